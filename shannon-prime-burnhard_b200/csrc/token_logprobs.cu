@@ -188,20 +188,27 @@ struct Seen {
     static constexpr int V = 16 / sizeof(T);
     uint64_t z = 0, a = 0;  // pairs of sums
     float m = -3.402823466e38f, limit = -3.402823466e38f;  // the maximum in use, and when to move it
-    float shift = 0.f;  // -m c, where products with c stay finite
+    // -m c rounded. Where `plain` the terms are x c + shift = t + rest(), one
+    // operation a value, and sums() takes the rest out again; it is below 2^-5, for
+    // |m c| is below 2^20 (beyond it, and where products with c overflow, the terms
+    // are (x - m) c).
+    float shift = 0.f;
     bool plain = false;
     float best = -__builtin_huge_valf(), second = -__builtin_huge_valf();
     int best_vec = -1;
 
+    __device__ __forceinline__ float rest(float c) const { return plain ? __fmaf_rn(m, c, shift) : 0.f; }
     __device__ __forceinline__ void move(float to, float c) {
-        const float t = log2_term(m, to, c), f = pow2(t);
-        const uint64_t f2 = pair(f, f), t2 = pair(t, t);
-        a = fma2(fma2(z, t2, a), f2, 0);
-        z = fma2(z, f2, 0);
+        float t = log2_term(m, to, c) - rest(c);
         m = to;
         limit = to + 8.f / c;
         shift = -to * c;
-        plain = fabsf(to) * c < 1e30f && fabsf(to) < (std::is_same<T, __half>::value ? 3e4f : 1e30f);
+        plain = fabsf(to) * c < 0x1p20f && fabsf(to) < (std::is_same<T, __half>::value ? 3e4f : 1e30f);
+        t += rest(c);
+        const float f = pow2(t);
+        const uint64_t f2 = pair(f, f), t2 = pair(t, t);
+        a = fma2(fma2(z, t2, a), f2, 0);
+        z = fma2(z, f2, 0);
     }
     __device__ __forceinline__ void term(float t0, float t1) {
         const uint64_t e = pair(pow2(t0), pow2(t1));
@@ -249,11 +256,14 @@ struct Seen {
             for (int i = 0; i < N * V; i += 2) term(log2_term(x[i], m, c), log2_term(x[i + 1], m, c));
         }
     }
-    __device__ __forceinline__ Softmax sums() const {
+    __device__ __forceinline__ Softmax sums(float c) const {
         float z0, z1, a0, a1;
         unpair(z, z0, z1);
         unpair(a, a0, a1);
-        return Softmax{m, z0 + z1, a0 + a1};
+        // from the terms' t + rest to t: 2^-rest by its series, whose error the small rest hides
+        const float r = rest(c), y = r * -0.6931471805599453f;
+        const float f = __fmaf_rn(y, __fmaf_rn(y, __fmaf_rn(y, 1.f / 6.f, 0.5f), 1.f), 1.f);
+        return Softmax{m, (z0 + z1) * f, __fmaf_rn(z0 + z1, -r, a0 + a1) * f};
     }
 };
 
@@ -350,7 +360,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(const Log
         for (int u = 0; u < UNROLL; ++u)
             if (v + u * LP_THREADS < w1) seen.template add<1>(next + u, v + u * LP_THREADS, c);
     }
-    const Softmax s_own = seen.sums();
+    const Softmax s_own = seen.sums(c);
     Softmax s = s_own;
     if (lane == 0 && warp == 0) n_cand = 0;
     const int k = p.k;

@@ -1,0 +1,46 @@
+"""GPU: the serving-step operators at the ends of their ranges: temperatures
+and offsets of logits, long rows of small probabilities, drafts that are not
+finite, cache layouts and batches beyond one pass of a search.
+
+Tolerances come from the arithmetic, as in test_gpu_serving.py.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+from test_gpu_serving import BF16, F16, F32, check_logprobs, dt, gen, randn, ws  # noqa: F401 (ws is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# log probabilities
+# ---------------------------------------------------------------------------
+def logprobs_held_to_64_bits(ctx, bh, ws, logits, k, scale):
+    import torch
+
+    rows, vocab = logits.shape
+    tokens = torch.randint(0, vocab, (rows, 2), generator=gen(vocab), device="cuda", dtype=torch.int32)
+    r = bh.token_logprobs(ctx, ws, logits, tokens, k, scale)
+    check_logprobs(logits, tokens, r, k, scale)
+    assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("type_", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,vocab", [(3, 32768), (700, 4096)])
+@pytest.mark.parametrize("scale", [0.01, 20.0, 100.0, 1e4, 1e6])
+def test_logprobs_of_any_temperature(ctx, bh, ws, type_, rows, vocab, scale):
+    """Products of maximum and scale that fp32 does not hold to a part of a nat."""
+    logprobs_held_to_64_bits(ctx, bh, ws, randn(gen(vocab), rows, vocab, dtype=type_, scale=4.0), 8, scale)
+
+
+@pytest.mark.parametrize("type_,offset", [(F32, 1e3), (F32, -1e3), (F32, 1e5), (F32, -1e9), (F32, 1e30), (F16, 2e4), (F16, -5e4),
+                                          (BF16, 1e3), (BF16, -1e9), (BF16, 1e30)])
+@pytest.mark.parametrize("rows", [2, 700])
+def test_logprobs_of_logits_with_a_common_offset(ctx, bh, ws, type_, offset, rows):
+    x = randn(gen(9), rows, 8192, scale=3.0)
+    logprobs_held_to_64_bits(ctx, bh, ws, (x + offset).to(dt(type_)), 8, 1.0)
+    x[:] = offset  # all equal
+    logprobs_held_to_64_bits(ctx, bh, ws, x.to(dt(type_)), 8, 1.0)
