@@ -155,15 +155,16 @@ __device__ __forceinline__ void block_join(Softmax& s, Softmax* warps, int warp,
     for (int w = 0; w < LP_WARPS; ++w) s.z += warps[w].z, s.a += warps[w].a;
 }
 
-// Two values as floats; for sums where the maximum in use is far above both
-// -1e30 and the type's lowest value, -inf as a value so low that its probability
-// is 0 all the same (0 times -inf would make the entropy's sum NaN).
+// Two values as floats; for sums where the maximum in use is far above it, -inf
+// as a value so low that its probability is 0 all the same (0 times -inf would
+// make the entropy's sum NaN), and all of a bf16 row below it alike. Seen::move
+// says where that holds.
 template <typename T>
 __device__ __forceinline__ uint32_t lift(uint32_t u);
 template <>
 __device__ __forceinline__ uint32_t lift<__nv_bfloat16>(uint32_t u) {
     uint32_t r;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0xfcf0fcf0u));  // -1e37
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0xf680f680u));  // -2^110
     return r;
 }
 template <>
@@ -203,7 +204,10 @@ struct Seen {
         m = to;
         limit = to + 8.f / c;
         shift = -to * c;
-        plain = fabsf(to) * c < 0x1p20f && fabsf(to) < (std::is_same<T, __half>::value ? 3e4f : 1e30f);
+        // lifted values: their products with c finite, and their terms, below 2^20
+        // less 2^110 c, 0 (c = 2^17: a temperature of 1e-5)
+        plain = fabsf(to) * c < 0x1p20f && fabsf(to) < (std::is_same<T, __half>::value ? 3e4f : 1e30f) &&
+                (sizeof(T) == 4 || (c < 0x1p17f && c > 0x1p-80f));
         t += rest(c);
         const float f = pow2(t);
         const uint64_t f2 = pair(f, f), t2 = pair(t, t);

@@ -24,7 +24,16 @@ def logprobs_held_to_64_bits(ctx, bh, ws, logits, k, scale):
     rows, vocab = logits.shape
     tokens = torch.randint(0, vocab, (rows, 2), generator=gen(vocab), device="cuda", dtype=torch.int32)
     r = bh.token_logprobs(ctx, ws, logits, tokens, k, scale)
-    check_logprobs(logits, tokens, r, k, scale)
+
+    def out_of_range(got, ids):
+        """A log probability below what fp32 holds is -inf in it; here the 64-bit value takes its place."""
+        u = logits.double() * scale
+        exact = u.gather(1, ids.long()) - u.amax(1, keepdim=True)
+        below = (got == -math.inf) & exact.isfinite() & (exact < torch.finfo(torch.float32).min)
+        return torch.where(below, exact, got.double())
+
+    check_logprobs(logits, tokens, r._replace(logprob=out_of_range(r.logprob, tokens),
+                                              top_logprob=out_of_range(r.top_logprob, r.top_ids)), k, scale)
     assert ctx.status() == 0
 
 
@@ -44,3 +53,24 @@ def test_logprobs_of_logits_with_a_common_offset(ctx, bh, ws, type_, offset, row
     logprobs_held_to_64_bits(ctx, bh, ws, (x + offset).to(dt(type_)), 8, 1.0)
     x[:] = offset  # all equal
     logprobs_held_to_64_bits(ctx, bh, ws, x.to(dt(type_)), 8, 1.0)
+
+
+def masked_rows(type_, rows, vocab, fill, every):
+    """Rows at odd alignments, their values but every `every`-th replaced."""
+    import torch
+
+    x = randn(gen(vocab + every), rows, vocab + 1, dtype=type_, scale=3.0)[:, 1:]
+    x[:, torch.arange(vocab, device="cuda") % every != every // 2] = fill
+    return x
+
+
+@pytest.mark.parametrize("type_", [BF16, F16, F32])
+@pytest.mark.parametrize("fill", ["-inf", "lowest"])
+@pytest.mark.parametrize("scale", [11.0, 25.0, 100.0, 1e4, 1e6])
+def test_logprobs_of_masked_rows_at_low_temperatures(ctx, bh, ws, type_, fill, scale):
+    import torch
+
+    low = -math.inf if fill == "-inf" else torch.finfo(dt(type_)).min
+    for rows, every in ((3, 5), (3, 50257), (600, 7)):
+        logprobs_held_to_64_bits(ctx, bh, ws, masked_rows(type_, rows, 50257, low, every), 4, scale)
+    logprobs_held_to_64_bits(ctx, bh, ws, randn(gen(3), 5, 50258, dtype=type_, scale=3.0)[:, 1:], 4, scale)  # nothing masked
