@@ -204,10 +204,12 @@ struct Seen {
         m = to;
         limit = to + 8.f / c;
         shift = -to * c;
-        // lifted values: their products with c finite, and their terms, below 2^20
-        // less 2^110 c, 0 (c = 2^17: a temperature of 1e-5)
-        plain = fabsf(to) * c < 0x1p20f && fabsf(to) < (std::is_same<T, __half>::value ? 3e4f : 1e30f) &&
-                (sizeof(T) == 4 || (c < 0x1p17f && c > 0x1p-80f));
+        // lifted values: their products with c finite, and their terms 0: of bf16,
+        // below 2^20 less 2^110 c, of f16, below (30000 - 65504) c (c = 2^17: a
+        // temperature of 1e-5, 2^-7: of 180)
+        constexpr bool half = std::is_same<T, __half>::value;
+        plain = fabsf(to) * c < 0x1p20f && fabsf(to) < (half ? 3e4f : 1e30f) &&
+                (sizeof(T) == 4 || (c < 0x1p17f && c > (half ? 0x1p-7f : 0x1p-80f)));
         t += rest(c);
         const float f = pow2(t);
         const uint64_t f2 = pair(f, f), t2 = pair(t, t);

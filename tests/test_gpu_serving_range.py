@@ -74,3 +74,11 @@ def test_logprobs_of_masked_rows_at_low_temperatures(ctx, bh, ws, type_, fill, s
     for rows, every in ((3, 5), (3, 50257), (600, 7)):
         logprobs_held_to_64_bits(ctx, bh, ws, masked_rows(type_, rows, 50257, low, every), 4, scale)
     logprobs_held_to_64_bits(ctx, bh, ws, randn(gen(3), 5, 50258, dtype=type_, scale=3.0)[:, 1:], 4, scale)  # nothing masked
+
+
+@pytest.mark.parametrize("type_", [F16, BF16, F32])
+@pytest.mark.parametrize("scale", [1e-2, 1e-3, 1e-4, 1e-6, 1e-30])
+def test_logprobs_of_masked_rows_at_high_temperatures(ctx, bh, ws, type_, scale):
+    """What is -inf has no probability, however flat the others' distribution is."""
+    for rows, every in ((3, 5), (600, 7)):
+        logprobs_held_to_64_bits(ctx, bh, ws, masked_rows(type_, rows, 20011, -math.inf, every), 4, scale)
