@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(const Log
     const int row_i = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
     const T* row = static_cast<const T*>(p.logits) + (int64_t)row_i * p.row_stride;
     const int n = p.n_vocab;
-    const float c = p.scale * 1.4426950408889634f;
+    const float c = fminf(p.scale * 1.4426950408889634f, 3.402823466e38f);  // finite: 0 times c is 0
     // 16-byte vectors from the aligned address at or before the row
     const int shift = (int)((reinterpret_cast<uintptr_t>(row) % 16) / sizeof(T));
     const int n_vec = (n + shift + V - 1) / V;

@@ -82,3 +82,19 @@ def test_logprobs_of_masked_rows_at_high_temperatures(ctx, bh, ws, type_, scale)
     """What is -inf has no probability, however flat the others' distribution is."""
     for rows, every in ((3, 5), (600, 7)):
         logprobs_held_to_64_bits(ctx, bh, ws, masked_rows(type_, rows, 20011, -math.inf, every), 4, scale)
+
+
+@pytest.mark.parametrize("type_", [F32, F16, BF16])
+def test_logprobs_of_the_largest_scales(ctx, bh, ws, type_):
+    """Scales whose product with log2(e) passes fp32: the likeliest tokens share the row."""
+    import torch
+
+    x = randn(gen(4), 2, 5000, dtype=type_)
+    x[:, 77] = x[:, 4001] = 9.0
+    x[1, 300] = -math.inf
+    r = bh.token_logprobs(ctx, ws, x, torch.tensor([[77, 5], [4001, 300]], dtype=torch.int32, device="cuda"), 2, 3e38)
+    near = 16 * 2.0**-24
+    assert (r.logprob[:, 0] + math.log(2)).abs().max() <= near and (r.logprob[:, 1] == -math.inf).all()
+    assert (r.entropy - math.log(2)).abs().max() <= near
+    assert r.top_ids.tolist() == [[77, 4001]] * 2 and (r.top_logprob + math.log(2)).abs().max() <= near
+    assert ctx.status() == 0
