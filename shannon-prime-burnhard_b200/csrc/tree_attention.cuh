@@ -750,6 +750,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
         // hold one are zeroed here and added by themselves below.
         bool mend = false;
         if (drafts && !sees_all) {
+            sync();  // a warp may still be adding rows of the tile before
             if (tid < (TN + 31) / 32) sh.bad[tid] = 0;
             sync();
 #pragma unroll

@@ -10,7 +10,7 @@ import math
 
 import pytest
 
-from test_gpu_serving import BF16, F16, F32, check_logprobs, dt, gen, randn, ws  # noqa: F401 (ws is a fixture)
+from test_gpu_serving import BF16, F16, F32, TYPES, Batch, check_logprobs, dt, gen, randn, ws  # noqa: F401 (ws is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -97,4 +97,40 @@ def test_logprobs_of_the_largest_scales(ctx, bh, ws, type_):
     assert (r.logprob[:, 0] + math.log(2)).abs().max() <= near and (r.logprob[:, 1] == -math.inf).all()
     assert (r.entropy - math.log(2)).abs().max() <= near
     assert r.top_ids.tolist() == [[77, 4001]] * 2 and (r.top_logprob + math.log(2)).abs().max() <= near
+    assert ctx.status() == 0
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("act,cache_t", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("n_new,dim", [(33, 128), (64, 128), (64, 64), (40, 256)])
+def test_attention_of_many_drafts_that_are_not_finite(ctx, bh, ws, act, cache_t, bad, n_new, dim):
+    """Two drafts of three with one bad value of V each, over several tiles: a row
+    has it where it sees the draft, and all else as if that value were zero."""
+    import torch
+
+    b = Batch(bh, 21, [70, 3], [n_new, 9], 8, 2, dim, act, cache_t, 16)
+    lame = [(s, j, (5 * j) % 8) for s in range(2) for j in range(b.new[s]) if j % 3 != 1]
+    at = [(*b.slots(s)[b.ctx[s] + j], c) for s, j, c in lame]
+
+    def put(x):
+        for blk, o, c in at:
+            b.cache.v[blk, o, :, c] = x
+
+    put(0.0)
+    clean, lse0 = b.run(ctx, bh, ws, mask=b.mask(), return_lse=True)
+    b.check(clean, lse0, True)
+    for _ in range(3):
+        put(bad)
+        out, lse = b.run(ctx, bh, ws, mask=b.mask(), return_lse=True)
+        put(0.0)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        for s, j, c in lame:
+            for i in range(b.new[s]):
+                if b.mask_h[b.start[s] + i] >> j & 1:
+                    hit[b.start[s] + i, :, c] = True
+        assert not out[hit].isfinite().any()
+        b.check(torch.where(hit, clean, out), lse, True)
     assert ctx.status() == 0
