@@ -743,7 +743,9 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
         const int pos0 = cur.tile * TN;
         const uint32_t k_at = tiles_a + stage * 2 * S::TILE, v_at = k_at + S::TILE;
         const uint8_t* v_mem = tiles + stage * 2 * S::TILE + S::TILE;
-        const bool whole = sh.whole[stage], drafts = !whole && pos0 + TN > cur.w.ctx;
+        // drafts: by the lengths alone, the same in every warp also after a wait that
+        // ran out, when `whole` may not be: barriers depend on it
+        const bool whole = sh.whole[stage], drafts = pos0 + TN > cur.w.ctx;
 
         // A draft that some row does not see must not reach that row's sums:
         // the products would make NaN of 0 times an infinity. Rows of V that

@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS)
                 __syncwarp();
                 tm_fence_after();
                 const bool whole = *(volatile int*)&sh.whole[meta];
-                if (!whole && pos0 + TN > cur.w.ctx) {
+                if (pos0 + TN > cur.w.ctx) {  // by the lengths: barriers depend on it, also after a wait that ran out
                     // A draft that some row does not see must not reach that
                     // row's sums: the products would make NaN of 0 times an
                     // infinity. Rows of V that hold one become zero in the ring
