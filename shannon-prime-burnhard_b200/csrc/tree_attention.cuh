@@ -73,7 +73,9 @@ struct AttnShape {
     static constexpr int MT = 16 * MI * RG, WARPS = RG * KG, COMPUTE = WARPS * 32, THREADS = COMPUTE + 32;
     static constexpr int NS = F ? 1 : TA == TC ? 1 : TC == BH_F16 ? 2 : 3;  // parts of q kept in shared memory
     static constexpr bool EXACT = TA == BH_F32;
-    static constexpr float OFF = NS == 2 ? 12.f : 0.f;  // exponent added to the probabilities' f16 parts
+    // exponent added to probabilities that f16 holds, which would lose those below
+    // 2^-25 of the largest: a long row has much of its sum there
+    static constexpr float OFF = TC == BH_F16 ? 12.f : 0.f;
     static constexpr int NT = DP / 8;  // accumulator tiles of 8 values
     static constexpr int ROW = DP * (int)sizeof(C);
     // 16 positions a warp (8 of fp32), more of short rows: 32 KB of K and V in a stage (64 KB for 256 values)

@@ -47,7 +47,9 @@ struct WideShape {
     static constexpr int TC = TC_, DP = DP_, STREAMS = STREAMS_;
     using C = typename ValueOf<TC>::type;
     using T = C;
-    static constexpr float OFF = 0.f;
+    // exponent added to f16 probabilities (2^6, and 2^8 that the maximum in use may
+    // lag, of 2^16), so that what is above 2^-31 of the largest reaches the sums
+    static constexpr float OFF = TC == BH_F16 ? 6.f : 0.f;
     static constexpr int TN = 64 * STREAMS, MT = 128 * STREAMS;
     static constexpr int SOFT = 128 * STREAMS, THREADS = SOFT + 96, CTAS = 3 - STREAMS;
     static constexpr int ROW = DP * 2, TILE = TN * ROW, BLOCK = TN * 128;  // 64 values of every row make a block
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS)
                         }
                         tm_wait_st();
                     }
-                    const float base = m == NONE ? 0.f : m, shift = -base * rs;
+                    const float base = m == NONE ? 0.f : m, shift = S::OFF - base * rs;
                     const uint64_t rs2 = pair(rs, rs), shift2 = pair(shift, shift);
                     uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -764,7 +766,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS)
                 }
                 if (my < rows) {
                     if (!complete) slot[my] = top, slot[MT + my] = sum, slot[2 * MT + my] = rs;
-                    else if (p.lse) p.lse[(int64_t)my_tok * p.n_head + my_head] = log_sum(top, rs, 0.f, sum);
+                    else if (p.lse) p.lse[(int64_t)my_tok * p.n_head + my_head] = log_sum(top, rs, S::OFF, sum);
                 }
             }
             sync();  // the next query rows take their place

@@ -10,7 +10,7 @@ import math
 
 import pytest
 
-from test_gpu_serving import BF16, F16, F32, TYPES, Batch, check_logprobs, dt, gen, randn, ws  # noqa: F401 (ws is a fixture)
+from test_gpu_serving import BF16, F16, F32, TYPES, U, Batch, check_logprobs, dt, gen, randn, u_of, ws  # noqa: F401 (ws is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -133,4 +133,43 @@ def test_attention_of_many_drafts_that_are_not_finite(ctx, bh, ws, act, cache_t,
                     hit[b.start[s] + i, :, c] = True
         assert not out[hit].isfinite().any()
         b.check(torch.where(hit, clean, out), lse, True)
+    assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("act,cache_t", [(F16, F16), (F32, F16), (BF16, BF16)])
+@pytest.mark.parametrize("n_new,dim", [(1, 128), (4, 64), (8, 128), (64, 128), (64, 64), (2, 256)])
+def test_attention_keeps_the_mass_of_small_probabilities(ctx, bh, ws, act, cache_t, n_new, dim):
+    """One position has nearly all of the probability, 16000 others 2^-26 to
+    2^-27.5 of it each, and values 2^10 times as large."""
+    import torch
+
+    n = 16000
+    b = Batch(bh, 12, [n], [n_new], 4, 1, dim, act, cache_t, 16)
+    g = gen(13)
+    k, v = b.cache.k, b.cache.v
+    k.zero_()
+    # the score is k[0] + k[1]: the second part finer than the first one's rounding
+    k[..., 0] = -math.log(2) * (26.1 + 1.3 * torch.rand(k.shape[:3], generator=g, device="cuda"))
+    k[..., 1] = torch.rand(k.shape[:3], generator=g, device="cuda") * 0.03
+    v[:] = (512 + 512 * torch.rand(v.shape, generator=g, device="cuda")).to(v.dtype)
+    blk, o = b.slots(0)[5]
+    k[blk, o], v[blk, o] = 0, 0
+    b.q = torch.zeros_like(b.q)
+    b.q[..., :2] = 1
+    out = b.run(ctx, bh, ws, mask=b.mask(), scale=1.0)
+    at = b.slots(0)
+    i, j = torch.tensor([x for x, _ in at], device="cuda"), torch.tensor([y for _, y in at], device="cuda")
+    keys, vals = k[i, j, 0].double(), v[i, j, 0].double()
+    e = torch.exp(keys[:, 0] + keys[:, 1])
+    for t in range(n_new):
+        see = torch.ones(n + n_new, dtype=torch.bool, device="cuda")
+        see[n:] = torch.tensor([bool(b.mask_h[t] >> x & 1) for x in range(n_new)], device="cuda")
+        p = e * see
+        want = (p @ vals) / p.sum()
+        # the exponents' and sums' roundings; p's to 16 bits: a relative one, and where they are
+        # subnormal (parts of f16, the largest 2^7, of fp32 rows 2^12 at least) half of 2^-24 each, signs at random
+        near = want * (2 * 64 * U + 4 * math.sqrt(n) * U + u_of(act) * 2)
+        if cache_t == F16:
+            near = near + 4 * math.sqrt(n) * 2.0**-25 * 2.0 ** (-12 if act == F32 else -7) * 1024
+        assert ((out[t].double() - want).abs() <= near).all(), (t, float(((out[t].double() - want).abs() / near).max()))
     assert ctx.status() == 0
