@@ -622,36 +622,36 @@ def _type_of(t) -> int:
     return ty
 
 
-def _ints(t, n: int, name: str, bits: int = 32) -> int:
-    """Device pointer of a contiguous integer tensor of at least n values."""
+def _ints(t, n: int, name: str, device: int, bits: int = 32) -> int:
+    """Device pointer of a contiguous integer tensor of at least n values on the context's device."""
     if not _INTS:
         _load_types()
-    if _INTS.get(t.dtype) != bits or not t.is_cuda or t.numel() < n or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous int{bits} device tensor of {n} values is wanted, got "
+    if _INTS.get(t.dtype) != bits or t.get_device() != device or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int{bits} tensor of {n} values on cuda:{device} is wanted, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _floats(t, n: int, name: str) -> int | None:
+def _floats(t, n: int, name: str, device: int) -> int | None:
     if t is None:
         return None
-    if _type_of(t) != F32 or not t.is_cuda or not t.is_contiguous() or t.numel() < n:
-        raise ValueError(f"{name}: a contiguous float32 device tensor of {n} values is wanted, got "
+    if _type_of(t) != F32 or t.get_device() != device or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{name}: a contiguous float32 tensor of {n} values on cuda:{device} is wanted, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _rows(t, heads: int, dim: int, name: str) -> int:
-    """Row stride of a device tensor [rows, heads * dim] or [rows, heads, dim]
-    whose rows are dense."""
-    ok = t.is_cuda and t.dim() in (2, 3) and t.stride(-1) == 1
+def _rows(t, heads: int, dim: int, name: str, device: int) -> int:
+    """Row stride of a tensor [rows, heads * dim] or [rows, heads, dim] on the
+    context's device whose rows are dense."""
+    ok = t.get_device() == device and t.dim() in (2, 3) and t.stride(-1) == 1
     if ok and t.dim() == 3:
         ok = t.shape[1] == heads and t.shape[2] == dim and (heads == 1 or t.stride(1) == dim)
     elif ok:
         ok = t.shape[1] == heads * dim
     if not ok:
-        raise ValueError(f"{name}: dense device rows of {heads} heads of {dim} are wanted, got {tuple(t.shape)} with "
-                         f"strides {t.stride()} on {t.device}")
+        raise ValueError(f"{name}: dense rows of {heads} heads of {dim} on cuda:{device} are wanted, got {tuple(t.shape)} "
+                         f"with strides {t.stride()} on {t.device}")
     return t.stride(0) if t.shape[0] > 1 else heads * dim
 
 
@@ -691,14 +691,20 @@ class PagedKV:
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
             raise ValueError("k and v: [n_blocks, block_size, n_head_kv, head_dim] of one shape, type and strides, "
                              f"values contiguous; got {tuple(k.shape)} {k.stride()} and {tuple(v.shape)} {v.stride()}")
-        if not (k.is_cuda and v.is_cuda):
-            raise ValueError("k and v are device tensors")
-        self.k, self.v = k, v
+        if not k.is_cuda or k.device != v.device:
+            raise ValueError("k and v are tensors of one device")
+        self.k, self.v, self.device = k, v, k.get_device()
         n_blocks, block, heads, dim = k.shape
         self.block_size, self.n_head_kv, self.head_dim = block, heads, dim
         self.struct = PagedKVStruct(k.data_ptr(), v.data_ptr(), _type_of(k), heads, dim, n_blocks, block, k.stride(0),
                                     k.stride(1), k.stride(2))
         self.ref = C.byref(self.struct)
+
+    def on(self, ctx: Context):
+        """The bh_paged_kv for a call of this context."""
+        if self.device != ctx.device:
+            raise ValueError(f"the cache is on cuda:{self.device}, the context on cuda:{ctx.device}")
+        return self.ref
 
 
 KVPlan = collections.namedtuple("KVPlan", "q_start seq pos slot mask counts")
@@ -710,20 +716,21 @@ def kv_plan(ctx: Context, ctx_lens, new_lens, free_blocks, block_tables, block_s
     max_blocks] is extended in place from free_blocks; returns the packed
     tokens' (q_start [n_seq + 1], seq, pos, slot, mask [n_tok], counts [2])."""
     n_seq, max_blocks = block_tables.shape
-    tables = _ints(block_tables, 0, "block_tables")
+    d = ctx.device
+    tables = _ints(block_tables, 0, "block_tables", d)
     if out is None:
         import torch
 
         i32, i64 = block_tables.new_empty, torch.int64
         out = KVPlan(i32(n_seq + 1), i32(n_tok), i32(n_tok), i32(n_tok, dtype=i64), i32(n_tok, dtype=i64), i32(2))
-    _check(lib.bh_kv_plan(ctx.h, _ints(ctx_lens, n_seq, "ctx_lens"), _ints(new_lens, n_seq, "new_lens"), n_seq,
-                          None if parents is None else _ints(parents, n_tok, "parents"),
-                          _ints(free_blocks, 0, "free_blocks"), free_blocks.numel(),
+    _check(lib.bh_kv_plan(ctx.h, _ints(ctx_lens, n_seq, "ctx_lens", d), _ints(new_lens, n_seq, "new_lens", d), n_seq,
+                          None if parents is None else _ints(parents, n_tok, "parents", d),
+                          _ints(free_blocks, 0, "free_blocks", d), free_blocks.numel(),
                           tables, max_blocks, block_size, n_tok,
-                          _ints(out.q_start, n_seq + 1, "q_start"), _ints(out.seq, n_tok, "seq"),
-                          _ints(out.pos, n_tok, "pos"), _ints(out.slot, n_tok, "slot", 64),
-                          None if out.mask is None else _ints(out.mask, n_tok, "mask", 64),
-                          _ints(out.counts, 2, "counts"), _stream_on(stream, ctx.device)), "bh_kv_plan")
+                          _ints(out.q_start, n_seq + 1, "q_start", d), _ints(out.seq, n_tok, "seq", d),
+                          _ints(out.pos, n_tok, "pos", d), _ints(out.slot, n_tok, "slot", d, 64),
+                          None if out.mask is None else _ints(out.mask, n_tok, "mask", d, 64),
+                          _ints(out.counts, 2, "counts", d), _stream_on(stream, d)), "bh_kv_plan")
     return out
 
 
@@ -743,18 +750,18 @@ def qk_norm_rope_append(ctx: Context, qkv, n_head: int, cache: PagedKV, rope, po
     """Per-head RMSNorm and rotation of projected q|k|v rows, k and v appended
     to the cache at their slots (bh_qk_norm_rope_append); returns q [n_tok,
     n_head, head_dim]. rope [n_pos, rot_dim / 2, 2] fp32, or None."""
-    n_tok, dim = qkv.shape[0], cache.head_dim
-    stride = _rows(qkv, n_head + 2 * cache.n_head_kv, dim, "qkv")
+    n_tok, dim, d = qkv.shape[0], cache.head_dim, ctx.device
+    stride = _rows(qkv, n_head + 2 * cache.n_head_kv, dim, "qkv", d)
     if q_out is None:
         q_out = qkv.new_empty((n_tok, n_head, dim))
     elif q_out.dtype != qkv.dtype or q_out.shape[0] < n_tok:
         raise ValueError("q_out: rows of qkv's type are wanted")
     n_pos, rot = (0, 0) if rope is None else (rope.shape[0], 2 * rope.shape[1])
-    _check(lib.bh_qk_norm_rope_append(ctx.h, qkv.data_ptr(), _type_of(qkv), n_tok, stride, n_head, cache.ref,
-                                      _floats(q_norm, dim, "q_norm"), _floats(k_norm, dim, "k_norm"), eps,
-                                      _floats(rope, n_pos * rot, "rope"), n_pos, rot, int(neox),
-                                      _ints(pos, n_tok, "pos"), _ints(slot, n_tok, "slot", 64), q_out.data_ptr(),
-                                      _rows(q_out, n_head, dim, "q_out"), _stream_on(stream, ctx.device)), "bh_qk_norm_rope_append")
+    _check(lib.bh_qk_norm_rope_append(ctx.h, qkv.data_ptr(), _type_of(qkv), n_tok, stride, n_head, cache.on(ctx),
+                                      _floats(q_norm, dim, "q_norm", d), _floats(k_norm, dim, "k_norm", d), eps,
+                                      _floats(rope, n_pos * rot, "rope", d), n_pos, rot, int(neox),
+                                      _ints(pos, n_tok, "pos", d), _ints(slot, n_tok, "slot", d, 64), q_out.data_ptr(),
+                                      _rows(q_out, n_head, dim, "q_out", d), _stream_on(stream, d)), "bh_qk_norm_rope_append")
     return q_out
 
 
@@ -766,7 +773,8 @@ def tree_attention(ctx: Context, ws: Workspace, q, cache: PagedKV, block_tables,
     [n_tok, n_head])."""
     n_tok, n_head, dim = q.shape
     n_seq, max_blocks = block_tables.shape
-    stride = _rows(q, n_head, cache.head_dim, "q")
+    d = ctx.device
+    stride = _rows(q, n_head, cache.head_dim, "q", d)
     if out is None:
         out = q.new_empty((n_tok, n_head, dim))
     elif out.dtype != q.dtype or out.shape[0] < n_tok:
@@ -776,12 +784,12 @@ def tree_attention(ctx: Context, ws: Workspace, q, cache: PagedKV, block_tables,
         import torch
 
         lse = q.new_empty((n_tok, n_head), dtype=torch.float32)
-    _check(lib.bh_tree_attention(ctx.h, ws.h, q.data_ptr(), _type_of(q), n_tok, stride, n_head, cache.ref,
-                                 _ints(block_tables, 0, "block_tables"), max_blocks, _ints(ctx_lens, n_seq, "ctx_lens"),
-                                 _ints(q_start, n_seq + 1, "q_start"), n_seq, max_new,
-                                 None if mask is None else _ints(mask, n_tok, "mask", 64),
+    _check(lib.bh_tree_attention(ctx.h, ws.h, q.data_ptr(), _type_of(q), n_tok, stride, n_head, cache.on(ctx),
+                                 _ints(block_tables, 0, "block_tables", d), max_blocks, _ints(ctx_lens, n_seq, "ctx_lens", d),
+                                 _ints(q_start, n_seq + 1, "q_start", d), n_seq, max_new,
+                                 None if mask is None else _ints(mask, n_tok, "mask", d, 64),
                                  dim**-0.5 if scale is None else scale, out.data_ptr(),
-                                 _rows(out, n_head, dim, "out"), _dp(lse), _stream_on(stream, ctx.device)), "bh_tree_attention")
+                                 _rows(out, n_head, dim, "out", d), _dp(lse), _stream_on(stream, d)), "bh_tree_attention")
     return (out, lse) if return_lse else out
 
 
@@ -796,15 +804,16 @@ def token_logprobs(ctx: Context, ws: Workspace, logits, tokens=None, k: int = 0,
     import torch
 
     rows, vocab = logits.shape
-    if not logits.is_cuda or (vocab > 1 and logits.stride(1) != 1):
-        raise ValueError("logits: device rows of contiguous values are wanted")
+    d = ctx.device
+    if logits.get_device() != d or (vocab > 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits: rows of contiguous values on cuda:{d} are wanted, got strides {logits.stride()} on {logits.device}")
     n = 0 if tokens is None else tokens.shape[1] if tokens.dim() == 2 else 1
     new, f32 = logits.new_empty, torch.float32
     r = TokenLogprobs(new((rows, n), dtype=f32), new(rows, dtype=f32), new((rows, k), dtype=torch.int32),
                       new((rows, k), dtype=f32))
     _check(lib.bh_token_logprobs(ctx.h, ws.h, logits.data_ptr(), _type_of(logits), rows, vocab,
                                  logits.stride(0) if rows > 1 else vocab, scale,
-                                 None if tokens is None else _ints(tokens, rows * n, "tokens"), n, r.logprob.data_ptr(),
+                                 None if tokens is None else _ints(tokens, rows * n, "tokens", d), n, r.logprob.data_ptr(),
                                  r.entropy.data_ptr(), k, r.top_ids.data_ptr(), r.top_logprob.data_ptr(),
                                  _stream_on(stream, ctx.device)), "bh_token_logprobs")
     return r
