@@ -655,6 +655,24 @@ def _rows(t, heads: int, dim: int, name: str, device: int) -> int:
     return t.stride(0) if t.shape[0] > 1 else heads * dim
 
 
+def _made_for(stream, device: int, make) -> tuple:
+    """make()'s tensors, the outputs of a call on `stream`. Those of another
+    stream than the current one come from that stream's memory: a block that
+    the current one freed may have kernels before it still. They outlive what
+    the current stream has been given to do when they are freed."""
+    if stream is None or _stream_on(stream, device) == _stream_on(None, device):
+        return make()
+    import torch
+
+    current, handle = torch.cuda.current_stream(device), _stream_on(stream, device)
+    side = torch.cuda.ExternalStream(handle, device) if handle else torch.cuda.default_stream(device)
+    with torch.cuda.stream(side):
+        made = make()
+    for t in made:
+        t.record_stream(current)
+    return made
+
+
 class Workspace:
     """The memory that tree_attention and token_logprobs join split rows in
     (bh_workspace): one for each stream whose calls may run at the same time."""
@@ -722,7 +740,8 @@ def kv_plan(ctx: Context, ctx_lens, new_lens, free_blocks, block_tables, block_s
         import torch
 
         i32, i64 = block_tables.new_empty, torch.int64
-        out = KVPlan(i32(n_seq + 1), i32(n_tok), i32(n_tok), i32(n_tok, dtype=i64), i32(n_tok, dtype=i64), i32(2))
+        out = _made_for(stream, d, lambda: KVPlan(i32(n_seq + 1), i32(n_tok), i32(n_tok), i32(n_tok, dtype=i64),
+                                                  i32(n_tok, dtype=i64), i32(2)))
     _check(lib.bh_kv_plan(ctx.h, _ints(ctx_lens, n_seq, "ctx_lens", d), _ints(new_lens, n_seq, "new_lens", d), n_seq,
                           None if parents is None else _ints(parents, n_tok, "parents", d),
                           _ints(free_blocks, 0, "free_blocks", d), free_blocks.numel(),
@@ -753,7 +772,7 @@ def qk_norm_rope_append(ctx: Context, qkv, n_head: int, cache: PagedKV, rope, po
     n_tok, dim, d = qkv.shape[0], cache.head_dim, ctx.device
     stride = _rows(qkv, n_head + 2 * cache.n_head_kv, dim, "qkv", d)
     if q_out is None:
-        q_out = qkv.new_empty((n_tok, n_head, dim))
+        q_out, = _made_for(stream, d, lambda: (qkv.new_empty((n_tok, n_head, dim)),))
     elif q_out.dtype != qkv.dtype or q_out.shape[0] < n_tok:
         raise ValueError("q_out: rows of qkv's type are wanted")
     n_pos, rot = (0, 0) if rope is None else (rope.shape[0], 2 * rope.shape[1])
@@ -776,14 +795,14 @@ def tree_attention(ctx: Context, ws: Workspace, q, cache: PagedKV, block_tables,
     d = ctx.device
     stride = _rows(q, n_head, cache.head_dim, "q", d)
     if out is None:
-        out = q.new_empty((n_tok, n_head, dim))
+        out, = _made_for(stream, d, lambda: (q.new_empty((n_tok, n_head, dim)),))
     elif out.dtype != q.dtype or out.shape[0] < n_tok:
         raise ValueError("out: rows of q's type are wanted")
     lse = None
     if return_lse:
         import torch
 
-        lse = q.new_empty((n_tok, n_head), dtype=torch.float32)
+        lse, = _made_for(stream, d, lambda: (q.new_empty((n_tok, n_head), dtype=torch.float32),))
     _check(lib.bh_tree_attention(ctx.h, ws.h, q.data_ptr(), _type_of(q), n_tok, stride, n_head, cache.on(ctx),
                                  _ints(block_tables, 0, "block_tables", d), max_blocks, _ints(ctx_lens, n_seq, "ctx_lens", d),
                                  _ints(q_start, n_seq + 1, "q_start", d), n_seq, max_new,
@@ -809,8 +828,8 @@ def token_logprobs(ctx: Context, ws: Workspace, logits, tokens=None, k: int = 0,
         raise ValueError(f"logits: rows of contiguous values on cuda:{d} are wanted, got strides {logits.stride()} on {logits.device}")
     n = 0 if tokens is None else tokens.shape[1] if tokens.dim() == 2 else 1
     new, f32 = logits.new_empty, torch.float32
-    r = TokenLogprobs(new((rows, n), dtype=f32), new(rows, dtype=f32), new((rows, k), dtype=torch.int32),
-                      new((rows, k), dtype=f32))
+    r = _made_for(stream, d, lambda: TokenLogprobs(new((rows, n), dtype=f32), new(rows, dtype=f32),
+                                                   new((rows, k), dtype=torch.int32), new((rows, k), dtype=f32)))
     _check(lib.bh_token_logprobs(ctx.h, ws.h, logits.data_ptr(), _type_of(logits), rows, vocab,
                                  logits.stride(0) if rows > 1 else vocab, scale,
                                  None if tokens is None else _ints(tokens, rows * n, "tokens", d), n, r.logprob.data_ptr(),

@@ -10,7 +10,8 @@ import math
 
 import pytest
 
-from test_gpu_serving import BF16, F16, F32, TYPES, U, Batch, check_logprobs, dt, gen, randn, u_of, ws  # noqa: F401 (ws is a fixture)
+from test_gpu_serving import (BF16, F16, F32, TYPES, U, Batch, check_logprobs, dt, gen, i32, i64, randn, u_of,
+                              ws)  # noqa: F401 (ws is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -172,4 +173,36 @@ def test_attention_keeps_the_mass_of_small_probabilities(ctx, bh, ws, act, cache
         if cache_t == F16:
             near = near + 4 * math.sqrt(n) * 2.0**-25 * 2.0 ** (-12 if act == F32 else -7) * 1024
         assert ((out[t].double() - want).abs() <= near).all(), (t, float(((out[t].double() - want).abs() / near).max()))
+    assert ctx.status() == 0
+
+
+# ---------------------------------------------------------------------------
+# streams
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("as_handle", [False, True])
+def test_outputs_on_another_stream_are_not_memory_that_the_current_one_still_writes(ctx, bh, ws, as_handle):
+    import torch
+
+    b = Batch(bh, 30, [40, 90], [2, 3], 4, 2, 64, BF16, BF16, 16)
+    logits, tokens = randn(gen(31), 6, 5000), i32([1, 2, 3, 4, 5, 6])
+    tables, free, lens, new = i32([[0, 1, -1], [2, 3, -1]]), i32([7, 8, 9]), i32([20, 31]), i32([2, 3])
+    qkv, rope, pos, slot = randn(gen(32), 5, 8 * 64, dtype=BF16), bh.rope_table(99, 64), i32([1, 2, 3, 4, 5]), i64([1, 2, 3, 4, 5])
+    calls = [lambda **kw: bh.kv_plan(ctx, lens, new, free, tables, 16, 5, **kw),
+             lambda **kw: (bh.qk_norm_rope_append(ctx, qkv, 4, b.cache, rope, pos, slot, **kw),),
+             lambda **kw: b.run(ctx, bh, ws, return_lse=True, **kw),
+             lambda **kw: bh.token_logprobs(ctx, ws, logits, tokens, 3, **kw)]
+    side = torch.cuda.Stream()
+    for call in calls:
+        want = [t.clone() for t in call()]
+        torch.cuda.synchronize()
+        old = [torch.empty_like(t) for t in want]
+        torch.cuda._sleep(20_000_000)  # about 10 ms, before the current stream writes the blocks that it frees
+        for t in old:
+            t.fill_(7)
+        del old, t
+        got = call(stream=side.cuda_stream if as_handle else side)
+        side.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
     assert ctx.status() == 0

@@ -30,6 +30,12 @@ def on(index, t):
     return t
 
 
+@pytest.fixture(autouse=True)
+def default_stream(bh, monkeypatch):
+    """Without a GPU there is no current stream to ask for."""
+    monkeypatch.setattr(bh, "_raw_stream", lambda device: 0)
+
+
 CTX = types.SimpleNamespace(h=None, device=0)
 WS = types.SimpleNamespace(h=None)
 
