@@ -775,6 +775,8 @@ def qk_norm_rope_append(ctx: Context, qkv, n_head: int, cache: PagedKV, rope, po
         q_out, = _made_for(stream, d, lambda: (qkv.new_empty((n_tok, n_head, dim)),))
     elif q_out.dtype != qkv.dtype or q_out.shape[0] < n_tok:
         raise ValueError("q_out: rows of qkv's type are wanted")
+    if rope is not None and (rope.dim() != 3 or rope.shape[2] != 2):
+        raise ValueError(f"rope: (cos, sin) rows [n_pos, rot_dim / 2, 2] are wanted, got {tuple(rope.shape)}")
     n_pos, rot = (0, 0) if rope is None else (rope.shape[0], 2 * rope.shape[1])
     _check(lib.bh_qk_norm_rope_append(ctx.h, qkv.data_ptr(), _type_of(qkv), n_tok, stride, n_head, cache.on(ctx),
                                       _floats(q_norm, dim, "q_norm", d), _floats(k_norm, dim, "k_norm", d), eps,

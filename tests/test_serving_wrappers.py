@@ -87,3 +87,12 @@ def test_a_tensor_of_another_gpu_is_refused(bh, away):
 def test_a_cache_of_two_gpus_is_refused(bh):
     with pytest.raises(ValueError):
         bh.PagedKV(on(0, torch.zeros(4, 16, 2, 64)), on(1, torch.zeros(4, 16, 2, 64)))
+
+
+@pytest.mark.parametrize("shape", [(8, 64, 4), (8, 64), (16, 32, 2, 2)])
+def test_a_rotation_table_of_another_shape_is_refused(bh, shape):
+    """Also one with enough values, which would be read as other angles."""
+    cache = bh.PagedKV(on(0, torch.zeros(4, 16, 2, 64)), on(0, torch.zeros(4, 16, 2, 64)))
+    with pytest.raises(ValueError):
+        bh.qk_norm_rope_append(CTX, on(0, torch.zeros(3, 8 * 64)), 4, cache, on(0, torch.zeros(shape)), on(0, torch.zeros(3, dtype=torch.int32)),
+                               on(0, torch.zeros(3, dtype=torch.int64)), stream=0)
