@@ -64,13 +64,13 @@ struct AttnParams {
 
 constexpr int TA_MIN_TILES = 2;  // a CTA's least share of the line
 
-template <int TA_, int TC_, int DP_, int MI_, int RG_, int KG_>
+template <int TA_, int TC_, int DP_, int RG_, int KG_>
 struct AttnShape {
-    static constexpr int TA = TA_, TC = TC_, DP = DP_, MI = MI_, RG = RG_, KG = KG_;
+    static constexpr int TA = TA_, TC = TC_, DP = DP_, RG = RG_, KG = KG_;
     using T = typename ValueOf<TA>::type;
     using C = typename ValueOf<TC>::type;
     static constexpr bool F = TC == BH_F32;
-    static constexpr int MT = 16 * MI * RG, WARPS = RG * KG, COMPUTE = WARPS * 32, THREADS = COMPUTE + 32;
+    static constexpr int MT = 16 * RG, WARPS = RG * KG, COMPUTE = WARPS * 32, THREADS = COMPUTE + 32;
     static constexpr int NS = F ? 1 : TA == TC ? 1 : TC == BH_F16 ? 2 : 3;  // parts of q kept in shared memory
     static constexpr bool EXACT = TA == BH_F32;
     // exponent added to probabilities that f16 holds, which would lose those below
@@ -88,7 +88,7 @@ struct AttnShape {
     // CTAs an SM: three of two stages where 128 registers do, else two (three stages if they fit) or one
     static constexpr int MORE = 2048 + 64 * MT;  // static shared memory and the system's
     static constexpr int room(int stages) { return 228 * 1024 / (stages * 2 * TILE + SHARED_Q + MORE); }
-    static constexpr int CTAS = THREADS > 160 ? 1 : MI * NT <= 16 && room(2) >= 3 ? 3 : room(2) >= 2 ? 2 : 1;
+    static constexpr int CTAS = THREADS > 160 ? 1 : NT <= 16 && room(2) >= 3 ? 3 : room(2) >= 2 ? 2 : 1;
     static constexpr int STAGES = room(3) >= CTAS ? 3 : 2;
     static constexpr size_t BYTES = (size_t)STAGES * 2 * TILE + SHARED_Q;
     static constexpr int SLOT = MT * (DP + 4);  // floats of a partial result
@@ -616,7 +616,7 @@ template <class S>
 __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(const AttnParams p) {
     using T = typename S::T;
     using C = typename S::C;
-    constexpr int MT = S::MT, MI = S::MI, TN = S::TN, WN = S::WN, NT = S::NT, STAGES = S::STAGES, ROW = S::ROW;
+    constexpr int MT = S::MT, TN = S::TN, WN = S::WN, NT = S::NT, STAGES = S::STAGES, ROW = S::ROW;
     constexpr int SN = WN / 8;     // score tiles of a warp
     constexpr int CPR = ROW / 16;  // chunks of a row
     constexpr int NC = S::COMPUTE;
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
     Cursor cur = sh.first;
     auto sync = [] { named_bar(1, NC); };
 
-    float acc[MI][NT][4], m[MI][2], l[MI][2];
+    float acc[NT][4], m[2], l[2];
     bool fresh = true;  // a row tile begins
     bool sees_all = true;
     int stage = 0;
@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
     // lane's places in the query rows, K and V: the tile's offset and the step's chunk are added by xor
     const int ar = (lane & 7) + (lane & 8), ac = lane >> 4;              // A and V: rows, then chunks
     const int br = (lane & 7) + ((lane >> 4) << 3), bc = lane >> 3 & 1;  // K: chunks, then rows
-    const uint32_t q_lane = q_a + k_chunk<S>(rg * MI * 16 + ar, ac);
+    const uint32_t q_lane = q_a + k_chunk<S>(rg * 16 + ar, ac);
     const uint32_t k_lane = k_chunk<S>(kg * WN + br, bc), v_lane = v_chunk<S>(kg * WN + ar, ac);
 
     // tiles until the line position f1
@@ -731,13 +731,10 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
             sees_all = true;
 #pragma unroll
             for (int w = 0; w < S::WARPS; ++w) sees_all = sees_all && sh.sees_all[w];
+            m[0] = m[1] = NONE;
+            l[0] = l[1] = 0.f;
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi) {
-                m[mi][0] = m[mi][1] = NONE;
-                l[mi][0] = l[mi][1] = 0.f;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) acc[mi][n][0] = acc[mi][n][1] = acc[mi][n][2] = acc[mi][n][3] = 0.f;
-            }
+            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
             fresh = false;
         }
         ring_wait(sh, &sh.full[stage], turn, p.status);
@@ -792,34 +789,29 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
 
         // scores; with small parts or TF32 terms in accumulators of their own, even and odd steps apart
         constexpr int CH = S::F ? 3 : S::NS == 1 ? 1 : S::NS;
-        float sc[CH][MI][SN][4];
+        float sc[CH][SN][4];
         if constexpr (S::F) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                    for (int n = 0; n < SN; ++n) sc[c][mi][n][0] = sc[c][mi][n][1] = sc[c][mi][n][2] = sc[c][mi][n][3] = 0.f;
+                for (int n = 0; n < SN; ++n) sc[c][n][0] = sc[c][n][1] = sc[c][n][2] = sc[c][n][3] = 0.f;
             // 16 values of a head at a time: a lane's four consecutive ones are two pairs of contraction indexes
             const float* qf = reinterpret_cast<const float*>(q_mem);
             const float* kf = reinterpret_cast<const float*>(tiles + stage * 2 * S::TILE);
 #pragma unroll 4
             for (int d = 0; d < S::DP / 16; ++d) {
-                uint32_t ah[MI][2][4], al[MI][2][4];
-#pragma unroll
-                for (int mi = 0; mi < MI; ++mi) {
-                    const int r = (rg * MI + mi) * 16 + g;
-                    const float4 x = *reinterpret_cast<const float4*>(qf + k_chunk<S>(r, d * 4 + t4) / 4);
-                    const float4 y = *reinterpret_cast<const float4*>(qf + k_chunk<S>(r + 8, d * 4 + t4) / 4);
-                    split_tf32(x.x, ah[mi][0][0], al[mi][0][0]);
-                    split_tf32(y.x, ah[mi][0][1], al[mi][0][1]);
-                    split_tf32(x.y, ah[mi][0][2], al[mi][0][2]);
-                    split_tf32(y.y, ah[mi][0][3], al[mi][0][3]);
-                    split_tf32(x.z, ah[mi][1][0], al[mi][1][0]);
-                    split_tf32(y.z, ah[mi][1][1], al[mi][1][1]);
-                    split_tf32(x.w, ah[mi][1][2], al[mi][1][2]);
-                    split_tf32(y.w, ah[mi][1][3], al[mi][1][3]);
-                }
+                uint32_t ah[2][4], al[2][4];
+                const int r = rg * 16 + g;
+                const float4 x = *reinterpret_cast<const float4*>(qf + k_chunk<S>(r, d * 4 + t4) / 4);
+                const float4 y = *reinterpret_cast<const float4*>(qf + k_chunk<S>(r + 8, d * 4 + t4) / 4);
+                split_tf32(x.x, ah[0][0], al[0][0]);
+                split_tf32(y.x, ah[0][1], al[0][1]);
+                split_tf32(x.y, ah[0][2], al[0][2]);
+                split_tf32(y.y, ah[0][3], al[0][3]);
+                split_tf32(x.z, ah[1][0], al[1][0]);
+                split_tf32(y.z, ah[1][1], al[1][1]);
+                split_tf32(x.w, ah[1][2], al[1][2]);
+                split_tf32(y.w, ah[1][3], al[1][3]);
 #pragma unroll
                 for (int n = 0; n < SN; ++n) {
                     const float4 k4 = *reinterpret_cast<const float4*>(kf + k_chunk<S>(kg * WN + n * 8 + g, d * 4 + t4) / 4);
@@ -829,13 +821,11 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
                     split_tf32(k4.z, hi[2], lo[2]);
                     split_tf32(k4.w, hi[3], lo[3]);
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            mma_tf32(sc[2][mi][n], al[mi][j], hi[2 * j], hi[2 * j + 1]);
-                            mma_tf32(sc[2][mi][n], ah[mi][j], lo[2 * j], lo[2 * j + 1]);
-                            mma_tf32(sc[j][mi][n], ah[mi][j], hi[2 * j], hi[2 * j + 1]);
-                        }
+                    for (int j = 0; j < 2; ++j) {
+                        mma_tf32(sc[2][n], al[j], hi[2 * j], hi[2 * j + 1]);
+                        mma_tf32(sc[2][n], ah[j], lo[2 * j], lo[2 * j + 1]);
+                        mma_tf32(sc[j][n], ah[j], hi[2 * j], hi[2 * j + 1]);
+                    }
                 }
             }
         } else {
@@ -845,106 +835,96 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
 #pragma unroll
                 for (int n = 0; n < SN / 2; ++n) ldsm4(b[n], ((k_at + k_lane) ^ (d << 5)) + n * 16 * ROW);
 #pragma unroll
-                for (int part = 0; part < S::NS; ++part)
+                for (int part = 0; part < S::NS; ++part) {
+                    uint32_t a[4];
+                    ldsm4(a, (q_lane ^ (d << 5)) + part * MT * ROW);
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi) {
-                        uint32_t a[4];
-                        ldsm4(a, (q_lane ^ (d << 5)) + part * MT * ROW + mi * 16 * ROW);
-#pragma unroll
-                        for (int n = 0; n < SN / 2; ++n) {
-                            if (d == 0) {
-                                mma16_first<C>(sc[part][mi][2 * n], a, b[n][0], b[n][1]);
-                                mma16_first<C>(sc[part][mi][2 * n + 1], a, b[n][2], b[n][3]);
-                            } else {
-                                mma16<C>(sc[part][mi][2 * n], a, b[n][0], b[n][1]);
-                                mma16<C>(sc[part][mi][2 * n + 1], a, b[n][2], b[n][3]);
-                            }
+                    for (int n = 0; n < SN / 2; ++n) {
+                        if (d == 0) {
+                            mma16_first<C>(sc[part][2 * n], a, b[n][0], b[n][1]);
+                            mma16_first<C>(sc[part][2 * n + 1], a, b[n][2], b[n][3]);
+                        } else {
+                            mma16<C>(sc[part][2 * n], a, b[n][0], b[n][1]);
+                            mma16<C>(sc[part][2 * n + 1], a, b[n][2], b[n][3]);
                         }
                     }
+                }
             }
         }
-        float (&s)[MI][SN][4] = sc[0];
+        float (&s)[SN][4] = sc[0];
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
+        for (int n = 0; n < SN; ++n)
 #pragma unroll
-            for (int n = 0; n < SN; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (CH == 2) s[mi][n][e] += sc[CH - 1][mi][n][e];
-                    if constexpr (CH == 3) s[mi][n][e] += sc[CH - 2][mi][n][e] + sc[CH - 1][mi][n][e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (CH == 2) s[n][e] += sc[CH - 1][n][e];
+                if constexpr (CH == 3) s[n][e] += sc[CH - 2][n][e] + sc[CH - 1][n][e];
+            }
         // probabilities
-        float alpha[MI][2];
+        float alpha[2];
         bool grew = false;
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = (rg * MI + mi) * 16 + g + 8 * h;
-                const float rs = sh.row_scale[r];
-                float top = m[mi][h];
-                if (!whole) {
-                    const uint64_t mask = sh.mask[r];
-#pragma unroll
-                    for (int n = 0; n < SN; ++n)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int in = kg * WN + n * 8 + 2 * t4 + e, j = pos0 + in - cur.w.ctx;
-                            const bool see = (sh.valid[stage][in / 32] >> (in & 31) & 1) && (j < 0 || (j < 64 && (mask >> j & 1)));
-                            if (!see) s[mi][n][2 * h + e] = NONE;
-                        }
-                }
-#pragma unroll
-                for (int n = 0; n < SN; ++n) top = fmaxf(top, fmaxf(s[mi][n][2 * h], s[mi][n][2 * h + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float base = top == NONE ? 0.f : top;
-                alpha[mi][h] = ex2((m[mi][h] - base) * rs);
-                grew = grew || top > m[mi][h];
-                m[mi][h] = top;
-                const float shift = OFF - base * rs;
-                float sum = 0.f;
+        for (int h = 0; h < 2; ++h) {
+            const int r = rg * 16 + g + 8 * h;
+            const float rs = sh.row_scale[r];
+            float top = m[h];
+            if (!whole) {
+                const uint64_t mask = sh.mask[r];
 #pragma unroll
                 for (int n = 0; n < SN; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float& x = s[mi][n][2 * h + e];
-                        // exact differences where the sums are; one operation where a 16-bit result hides base's rounding
-                        x = ex2(S::EXACT ? __fmaf_rn(x - base, rs, OFF) : __fmaf_rn(x, rs, shift));
-                        sum += x;
+                        const int in = kg * WN + n * 8 + 2 * t4 + e, j = pos0 + in - cur.w.ctx;
+                        const bool see = (sh.valid[stage][in / 32] >> (in & 31) & 1) && (j < 0 || (j < 64 && (mask >> j & 1)));
+                        if (!see) s[n][2 * h + e] = NONE;
                     }
-                l[mi][h] = __fmaf_rn(l[mi][h], alpha[mi][h], sum);
             }
+#pragma unroll
+            for (int n = 0; n < SN; ++n) top = fmaxf(top, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float base = top == NONE ? 0.f : top;
+            alpha[h] = ex2((m[h] - base) * rs);
+            grew = grew || top > m[h];
+            m[h] = top;
+            const float shift = OFF - base * rs;
+            float sum = 0.f;
+#pragma unroll
+            for (int n = 0; n < SN; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float& x = s[n][2 * h + e];
+                    // exact differences where the sums are; one operation where a 16-bit result hides base's rounding
+                    x = ex2(S::EXACT ? __fmaf_rn(x - base, rs, OFF) : __fmaf_rn(x, rs, shift));
+                    sum += x;
+                }
+            l[h] = __fmaf_rn(l[h], alpha[h], sum);
+        }
         if constexpr (!S::EXACT) {
             if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            acc[mi][n][e] *= alpha[mi][e >> 1];
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        acc[n][e] *= alpha[e >> 1];
+                    }
             }
         }
         // the sums with V
         constexpr bool APART = S::EXACT;  // this tile's products by themselves
         if constexpr (S::F) {
             const float* vf = reinterpret_cast<const float*>(v_mem);
-            uint32_t ah[MI][SN][4], al[MI][SN][4];
+            uint32_t ah[SN][4], al[SN][4];
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                for (int n = 0; n < SN; ++n) {
-                    split_tf32(s[mi][n][0], ah[mi][n][0], al[mi][n][0]);
-                    split_tf32(s[mi][n][2], ah[mi][n][1], al[mi][n][1]);
-                    split_tf32(s[mi][n][1], ah[mi][n][2], al[mi][n][2]);
-                    split_tf32(s[mi][n][3], ah[mi][n][3], al[mi][n][3]);
-                }
+            for (int n = 0; n < SN; ++n) {
+                split_tf32(s[n][0], ah[n][0], al[n][0]);
+                split_tf32(s[n][2], ah[n][1], al[n][1]);
+                split_tf32(s[n][1], ah[n][2], al[n][2]);
+                split_tf32(s[n][3], ah[n][3], al[n][3]);
+            }
             // a lane's columns of four accumulator tiles are four consecutive values of V
 #pragma unroll
             for (int d = 0; d < S::DP / 32; ++d) {
-                float o[MI][4][4];
+                float o[4][4];
 #pragma unroll
                 for (int n = 0; n < SN; ++n) {
                     const int r = kg * WN + n * 8 + 2 * t4;
@@ -960,45 +940,39 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
                     split_tf32(y.z, yh[2], yl[2]);
                     split_tf32(y.w, yh[3], yl[3]);
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (n == 0) mma_tf32_first(o[mi][j], al[mi][n], xh[j], yh[j]);
-                            else mma_tf32(o[mi][j], al[mi][n], xh[j], yh[j]);
-                            mma_tf32(o[mi][j], ah[mi][n], xl[j], yl[j]);
-                            mma_tf32(o[mi][j], ah[mi][n], xh[j], yh[j]);
-                        }
+                    for (int j = 0; j < 4; ++j) {
+                        if (n == 0) mma_tf32_first(o[j], al[n], xh[j], yh[j]);
+                        else mma_tf32(o[j], al[n], xh[j], yh[j]);
+                        mma_tf32(o[j], ah[n], xl[j], yl[j]);
+                        mma_tf32(o[j], ah[n], xh[j], yh[j]);
+                    }
                 }
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            acc[mi][4 * d + j][e] = __fmaf_rn(acc[mi][4 * d + j][e], alpha[mi][e >> 1], o[mi][j][e]);
+                    for (int e = 0; e < 4; ++e)
+                        acc[4 * d + j][e] = __fmaf_rn(acc[4 * d + j][e], alpha[e >> 1], o[j][e]);
             }
         } else {
-            uint32_t a[MI][SN / 2][S::NS][4];
+            uint32_t a[SN / 2][S::NS][4];
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi)
+            for (int n = 0; n < SN / 2; ++n)
 #pragma unroll
-                for (int n = 0; n < SN / 2; ++n)
+                for (int i = 0; i < 4; ++i) {
+                    float x = s[2 * n + (i >> 1)][2 * (i & 1)], y = s[2 * n + (i >> 1)][2 * (i & 1) + 1];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float x = s[mi][2 * n + (i >> 1)][2 * (i & 1)], y = s[mi][2 * n + (i >> 1)][2 * (i & 1) + 1];
-#pragma unroll
-                        for (int part = 0; part < S::NS; ++part) {
-                            a[mi][n][part][i] = pack2<C>(x, y);
-                            if (part + 1 < S::NS) {
-                                float u, v;
-                                unpack2<C>(a[mi][n][part][i], u, v);
-                                x -= u, y -= v;
-                            }
+                    for (int part = 0; part < S::NS; ++part) {
+                        a[n][part][i] = pack2<C>(x, y);
+                        if (part + 1 < S::NS) {
+                            float u, v;
+                            unpack2<C>(a[n][part][i], u, v);
+                            x -= u, y -= v;
                         }
                     }
+                }
 #pragma unroll
             for (int d = 0; d < NT; d += 2) {
-                float o[APART ? MI : 1][2][4];
+                float o[2][4];
 #pragma unroll
                 for (int n = 0; n < SN / 2; ++n) {
                     uint32_t b[4];
@@ -1006,24 +980,20 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
 #pragma unroll
                     for (int part = S::NS - 1; part >= 0; --part)
 #pragma unroll
-                        for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                float (&to)[4] = APART ? o[APART ? mi : 0][j] : acc[mi][d + j];
-                                if (APART && n == 0 && part == S::NS - 1)
-                                    mma16_first<C>(to, a[mi][n][part], b[2 * j], b[2 * j + 1]);
-                                else
-                                    mma16<C>(to, a[mi][n][part], b[2 * j], b[2 * j + 1]);
-                            }
+                        for (int j = 0; j < 2; ++j) {
+                            float (&to)[4] = APART ? o[j] : acc[d + j];
+                            if (APART && n == 0 && part == S::NS - 1)
+                                mma16_first<C>(to, a[n][part], b[2 * j], b[2 * j + 1]);
+                            else
+                                mma16<C>(to, a[n][part], b[2 * j], b[2 * j + 1]);
+                        }
                 }
                 if constexpr (APART) {
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                acc[mi][d + j][e] = __fmaf_rn(acc[mi][d + j][e], alpha[mi][e >> 1], o[mi][j][e]);
+                        for (int e = 0; e < 4; ++e)
+                            acc[d + j][e] = __fmaf_rn(acc[d + j][e], alpha[e >> 1], o[j][e]);
                 }
             }
         }
@@ -1044,23 +1014,21 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
                                  (pos - blk * p.kv.block_size) * p.kv.token_stride + cur.head * p.kv.head_stride;
                     const int src = (lane & ~3) | (in & 7) >> 1;
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
+                    for (int h = 0; h < 2; ++h) {
+                        const float p0 = __shfl_sync(0xffffffffu, s[n][2 * h], src);
+                        const float p1 = __shfl_sync(0xffffffffu, s[n][2 * h + 1], src);
+                        const float pr = in & 1 ? p1 : p0;
+                        const int j = (int)pos - cur.w.ctx;
+                        if (j < 64 && (sh.mask[rg * 16 + g + 8 * h] >> j & 1)) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float p0 = __shfl_sync(0xffffffffu, s[mi][n][2 * h], src);
-                            const float p1 = __shfl_sync(0xffffffffu, s[mi][n][2 * h + 1], src);
-                            const float pr = in & 1 ? p1 : p0;
-                            const int j = (int)pos - cur.w.ctx;
-                            if (j < 64 && (sh.mask[(rg * MI + mi) * 16 + g + 8 * h] >> j & 1)) {
+                            for (int d = 0; d < NT; ++d)
 #pragma unroll
-                                for (int d = 0; d < NT; ++d)
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e)
-                                        if (dim_of(d, e) < p.dim)
-                                            acc[mi][d][2 * h + e] =
-                                                __fmaf_rn(pr, to_f32(v[dim_of(d, e)]), acc[mi][d][2 * h + e]);
-                            }
+                                for (int e = 0; e < 2; ++e)
+                                    if (dim_of(d, e) < p.dim)
+                                        acc[d][2 * h + e] =
+                                            __fmaf_rn(pr, to_f32(v[dim_of(d, e)]), acc[d][2 * h + e]);
                         }
+                    }
                 }
         }
 
@@ -1071,55 +1039,49 @@ __global__ void __launch_bounds__(S::THREADS, S::CTAS) tree_attention_kernel(con
             // join the position groups: maxima, then sums in their order
             float* epi = reinterpret_cast<float*>(q_mem);
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    l[mi][h] += __shfl_xor_sync(0xffffffffu, l[mi][h], 1);
-                    l[mi][h] += __shfl_xor_sync(0xffffffffu, l[mi][h], 2);
-                    const int r = (rg * MI + mi) * 16 + g + 8 * h;
-                    if (t4 == 0) sh.part_m[kg][r] = m[mi][h], sh.part_l[kg][r] = l[mi][h];
-                }
+            for (int h = 0; h < 2; ++h) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                const int r = rg * 16 + g + 8 * h;
+                if (t4 == 0) sh.part_m[kg][r] = m[h], sh.part_l[kg][r] = l[h];
+            }
             sync();
-            float f2[MI][2];
+            float f2[2];
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi)
+            for (int h = 0; h < 2; ++h) {
+                const int r = rg * 16 + g + 8 * h;
+                float top = sh.part_m[0][r];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = (rg * MI + mi) * 16 + g + 8 * h;
-                    float top = sh.part_m[0][r];
+                for (int k = 1; k < S::KG; ++k) top = fmaxf(top, sh.part_m[k][r]);
+                const float base = top == NONE ? 0.f : top;
+                const float rs = sh.row_scale[r];
+                f2[h] = ex2((m[h] - base) * rs);
+                if (kg == 0 && t4 == 0) {
+                    float sum = 0.f;
 #pragma unroll
-                    for (int k = 1; k < S::KG; ++k) top = fmaxf(top, sh.part_m[k][r]);
-                    const float base = top == NONE ? 0.f : top;
-                    const float rs = sh.row_scale[r];
-                    f2[mi][h] = ex2((m[mi][h] - base) * rs);
-                    if (kg == 0 && t4 == 0) {
-                        float sum = 0.f;
-#pragma unroll
-                        for (int k = 0; k < S::KG; ++k) sum += sh.part_l[k][r] * ex2((sh.part_m[k][r] - base) * rs);
-                        sh.row_m[r] = top;
-                        sh.row_l[r] = sum;
-                    }
+                    for (int k = 0; k < S::KG; ++k) sum += sh.part_l[k][r] * ex2((sh.part_m[k][r] - base) * rs);
+                    sh.row_m[r] = top;
+                    sh.row_l[r] = sum;
                 }
+            }
             // few rows: a place for every group; else one place, the groups in turn
             const bool side = rows * S::KG <= MT;
 #pragma unroll
             for (int k = 0; k < S::KG; ++k) {
                 if (kg == k) {
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = rg * 16 + g + 8 * h;
+                        if (r >= rows) continue;
+                        float* row = epi + (side ? k * rows + r : r) * S::DP;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int r = (rg * MI + mi) * 16 + g + 8 * h;
-                            if (r >= rows) continue;
-                            float* row = epi + (side ? k * rows + r : r) * S::DP;
+                        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const float x = acc[mi][n][2 * h + e] * f2[mi][h];
-                                    row[dim_of(n, e)] = k == 0 || side ? x : row[dim_of(n, e)] + x;
-                                }
-                        }
+                            for (int e = 0; e < 2; ++e) {
+                                const float x = acc[n][2 * h + e] * f2[h];
+                                row[dim_of(n, e)] = k == 0 || side ? x : row[dim_of(n, e)] + x;
+                            }
+                    }
                 }
                 if (!side && k + 1 < S::KG) sync();
             }
@@ -1185,11 +1147,11 @@ int launch_attention_shape(const AttnParams& p, int num_sms, cudaStream_t s) {
 template <int TA, int TC>
 int launch_attention(const AttnParams& p, int num_sms, cudaStream_t s) {
     const int rows = p.max_new * (p.n_head / p.n_kv);
-    if (p.dim <= 64) return launch_attention_shape<AttnShape<TA, TC, 64, 1, 1, 4>>(p, num_sms, s);
-    if (p.dim <= 128) return launch_attention_shape<AttnShape<TA, TC, 128, 1, 1, 4>>(p, num_sms, s);
-    if (rows <= 16) return launch_attention_shape<AttnShape<TA, TC, 256, 1, 1, 4>>(p, num_sms, s);
-    if (rows <= 32) return launch_attention_shape<AttnShape<TA, TC, 256, 1, 2, 2>>(p, num_sms, s);
-    return launch_attention_shape<AttnShape<TA, TC, 256, 1, 4, 2>>(p, num_sms, s);
+    if (p.dim <= 64) return launch_attention_shape<AttnShape<TA, TC, 64, 1, 4>>(p, num_sms, s);
+    if (p.dim <= 128) return launch_attention_shape<AttnShape<TA, TC, 128, 1, 4>>(p, num_sms, s);
+    if (rows <= 16) return launch_attention_shape<AttnShape<TA, TC, 256, 1, 4>>(p, num_sms, s);
+    if (rows <= 32) return launch_attention_shape<AttnShape<TA, TC, 256, 2, 2>>(p, num_sms, s);
+    return launch_attention_shape<AttnShape<TA, TC, 256, 4, 2>>(p, num_sms, s);
 }
 
 // one for each pair of types, in files of their own
