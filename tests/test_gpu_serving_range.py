@@ -206,3 +206,57 @@ def test_outputs_on_another_stream_are_not_memory_that_the_current_one_still_wri
         torch.cuda.synchronize()
         assert all(torch.equal(g, w) for g, w in zip(got, want))
     assert ctx.status() == 0
+
+
+# ---------------------------------------------------------------------------
+# many query rows: cache layouts, head sizes, long caches, many sequences
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("act", [F16, BF16])
+@pytest.mark.parametrize("new_lens", [[9, 30, 1], [64, 20, 40]])  # up to 128 rows of a head, and more
+@pytest.mark.parametrize("layout", ["token", "head", "padded"])
+@pytest.mark.parametrize("dim,block", [(128, 8), (128, 16), (64, 64), (64, 24), (72, 16), (80, 32), (96, 128), (104, 256), (120, 512), (8, 16),
+                                       (40, 8), (56, 48)])
+def test_attention_of_many_rows_over_cache_layouts(ctx, bh, ws, act, new_lens, layout, dim, block):
+    """Boxes of every size by tensor copies, heads that they reach beyond, and
+    values behind the heads that are not numbers."""
+    import torch
+
+    b = Batch(bh, dim + block, [700, 129, 1500], new_lens, 8, 2, dim, act, act, block, layout)
+    if layout == "padded":
+        for t in (b.cache.k, b.cache.v):
+            flat = torch.as_strided(t, (t.shape[0] * block * 3 * (dim + 16) - t.storage_offset(),), (1,), t.storage_offset())
+            keep = t.clone()
+            flat.fill_(math.nan)
+            t.copy_(keep)
+    out, lse = b.run(ctx, bh, ws, mask=b.mask(), return_lse=True)
+    b.check(out, lse, True)
+    assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("n_new", [8, 40])  # 32 and 160 rows of a head
+def test_attention_of_many_rows_beyond_32_bit_offsets(ctx, bh, ws, n_new):
+    import torch
+
+    block, heads, dim = 64, 8, 128
+    n_blocks = (1 << 31) // (block * heads * dim) + 40
+    k, v = (torch.empty((n_blocks, block, heads, dim), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    small = Batch(bh, 40, [100, 700], [n_new, 3], 32, heads, dim, BF16, BF16, block)
+    used = small.cache.k.shape[0]
+    k[-used:], v[-used:] = small.cache.k, small.cache.v
+    want = small.run(ctx, bh, ws, mask=small.mask())
+    small.check(want, None, True)
+    small.cache, small.tables = bh.PagedKV(k, v), torch.where(small.tables >= 0, small.tables + (n_blocks - used), -1)
+    assert torch.equal(small.run(ctx, bh, ws, mask=small.mask()), want)
+    assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("act,cache_t", TYPES)
+@pytest.mark.parametrize("n_seq", [353, 900])  # more than any kernel has threads
+@pytest.mark.parametrize("group", [1, 16])
+def test_attention_of_many_sequences(ctx, bh, ws, act, cache_t, n_seq, group):
+    new = [(7 * i) % 4 for i in range(n_seq)]
+    new[3], new[-1] = 9, 5
+    b = Batch(bh, n_seq, [(i * 37) % 150 if i % 11 else 600 for i in range(n_seq)], new, group, 1, 64, act, cache_t, 16)
+    out, lse = b.run(ctx, bh, ws, mask=b.mask(), return_lse=True)
+    b.check(out, lse, True)
+    assert ctx.status() == 0
