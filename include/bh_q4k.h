@@ -564,9 +564,11 @@ int bh_gguf_get_str(const bh_gguf *g, int64_t k, const char **s, uint64_t *len);
  * and read on the stream: no call of a step waits for the device, and a step
  * with buffers of a fixed size can be captured in a CUDA graph. What the
  * device finds wrong (a position outside the rotation table, a block id or a
- * slot outside the cache, a sequence longer than its table or than max_new)
- * is never read or written: it sets the context's status word
- * (bh_device_status: BH_EINVAL) and is left out of the result.
+ * slot outside the cache, bh_tree_attention's sequences that are longer than
+ * their table or than max_new) is never read or written: it sets the context's
+ * status word (bh_device_status: BH_EINVAL) and is left out of the result. To
+ * bh_kv_plan a sequence that its table or the free list has no block for is
+ * not an error: its tokens have slot -1, and nothing of them is stored.
  * ------------------------------------------------------------------------ */
 /* value types of activations, caches and logits */
 #define BH_F32 0
@@ -617,10 +619,12 @@ size_t bh_workspace_bytes(bh_workspace *ws);
  *   tok_pos [n_tok]      position: ctx + i for the i-th new token, or with
  *                        parents_opt ctx + its depth in the tree
  *   tok_slot [n_tok]     the cache slot of position ctx + i, -1 without a block
+ *                        (none left in the free list, or no column in the table)
  *   tok_mask_opt [n_tok] bit j: the sequence's new token j is the token itself
  *                        or (parents_opt) an ancestor of it, or (no parents) an
  *                        earlier one; bits exist for the first 64 tokens
- *   counts [2]           tokens, and blocks taken (more than n_free: too few)
+ *   counts [2]           tokens, and blocks taken, as many as the tables have
+ *                        room for (more than n_free: the free list has too few)
  * parents_opt [n_tok]: the parent's index among the sequence's new tokens, -1
  * for a child of the last cached token; a parent precedes its child, and a
  * sequence with parents has at most BH_TREE_MAX new tokens (else the status
@@ -660,12 +664,16 @@ int bh_qk_norm_rope_append(bh_ctx *ctx, const void *qkv, int act_type, int n_tok
  * h / (n_head / n_head_kv). Softmax of scale * q.k in 32 bits; out rows of
  * out_stride elements, lse_opt [n_tok][n_head] fp32 (natural log of the sum).
  * A row that sees nothing gives zeros and -inf; what a row does not see takes
- * no part in it, NaN and infinities included. act_type is the type of q and
- * out: the cache's own, or BH_F32 over any cache (then q and the probabilities
+ * no part in it, NaN and infinities included. A value of V that a row sees and
+ * that is not finite makes that value of its output an infinity or NaN, and no
+ * other; a key that is not finite may make the whole row NaN (fp32 rows enter
+ * the products in parts, and an infinity has none). act_type is the type of q
+ * and out: the cache's own (the probabilities are rounded to it for the
+ * products with V), or BH_F32 over any cache (then q and the probabilities
  * enter the products with more bits than the cache's type has). At most
  * max_new (<= BH_TREE_MAX) new tokens a sequence; rows outside every sequence
  * are not written. q and out are 16-byte aligned, strides multiples of 16
- * bytes. */
+ * bytes; out does not overlap q. */
 int bh_tree_attention(bh_ctx *ctx, bh_workspace *ws, const void *q, int act_type, int n_tok, int64_t q_stride,
                       int n_head, const bh_paged_kv *kv, const int32_t *block_tables, int max_blocks,
                       const int32_t *ctx_lens, const int32_t *q_start, int n_seq, int max_new,

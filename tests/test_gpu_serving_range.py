@@ -260,3 +260,33 @@ def test_attention_of_many_sequences(ctx, bh, ws, act, cache_t, n_seq, group):
     out, lse = b.run(ctx, bh, ws, mask=b.mask(), return_lse=True)
     b.check(out, lse, True)
     assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("act,cache_t", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("new_lens", [[1, 2], [30, 9], [64, 3]])
+def test_attention_of_history_that_is_not_finite(ctx, bh, ws, act, cache_t, bad, new_lens):
+    """A value of V shows in that value of the output and in no other, a key in
+    its sequence's rows of its KV head and in no others."""
+    import torch
+
+    b = Batch(bh, 50, [400, 90], new_lens, 8, 2, 128, act, cache_t, 16)
+    at = [b.slots(0)[17], b.slots(0)[333]]
+    for (blk, o), c in zip(at, (5, 100)):
+        b.cache.v[blk, o, 1, c] = 0
+    clean, lse0 = b.run(ctx, bh, ws, mask=b.mask(), return_lse=True)
+    b.check(clean, lse0, True)
+    for (blk, o), c in zip(at, (5, 100)):
+        b.cache.v[blk, o, 1, c] = bad
+    out, lse = b.run(ctx, bh, ws, mask=b.mask(), return_lse=True)
+    n = new_lens[0]
+    assert not out[:n, 4:, [5, 100]].isfinite().any()
+    out[:n, 4:, [5, 100]] = clean[:n, 4:, [5, 100]]
+    assert torch.equal(out, clean) and torch.equal(lse, lse0)
+    for (blk, o), c in zip(at, (5, 100)):
+        b.cache.v[blk, o, 1, c] = 0
+    b.cache.k[at[0][0], at[0][1], 1, 64] = bad
+    out, lse = b.run(ctx, bh, ws, mask=b.mask(), return_lse=True)
+    out[:n, 4:], lse[:n, 4:] = clean[:n, 4:], lse0[:n, 4:]
+    assert torch.equal(out, clean) and torch.equal(lse, lse0)
+    assert ctx.status() == 0
