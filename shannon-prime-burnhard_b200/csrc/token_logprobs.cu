@@ -537,8 +537,8 @@ extern "C" int bh_token_logprobs(bh_ctx* ctx, bh_workspace* ws, const void* logi
     // Rows are split until the machine is full (four CTAs an SM), parts of at
     // least four vectors a thread: the number that makes the waves of CTAs, each
     // as long as its bytes and an end worth about 96 KB of them, the shortest
-    // (2048 rows of 304 KB: 144 us unsplit, 182 in halves; 8 rows of 608 KB: 10.7
-    // us in 37 parts, 12.5 in 74).
+    // (2048 rows of 304 KB: 122 us unsplit, 157 in halves; 8 rows of 608 KB: 10.7
+    // us in 37 parts, 12.8 in 74, 15.7 unsplit).
     const int64_t bytes = (int64_t)n_vocab * bh::type_bytes(type), room = (int64_t)ctx->num_sms * 4;
     const int64_t most = bytes / 16 / (bh::LP_THREADS * 4);
     int64_t splits = 1, least = INT64_MAX;
