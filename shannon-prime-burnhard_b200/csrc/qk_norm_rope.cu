@@ -16,9 +16,9 @@
 //
 // Measured in a graph, 32 + 8 + 8 heads of 128 values: one token 3.1 us (launch
 // and two dependent loads); 509 tokens of fp32 into an f16 cache 6.5 us, 3.5
-// TB/s from the L2; 16384 of bf16 88 us, 4.65 TB/s, where conversions, norm and
-// rotation keep the arithmetic units as busy as the memory (fp32 throughout, the
-// same bytes a value and half the work a byte, 5.9 TB/s).
+// TB/s from the L2; 16384 of bf16 88 us, 4.65 TB/s, where warps wait for loads
+// with the issue slots 43% busy: 64 bytes a lane are in flight (fp32 throughout,
+// with 128 bytes a lane, 5.9 TB/s).
 #include "paged_kv.cuh"
 
 namespace bh {
