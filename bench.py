@@ -408,7 +408,11 @@ def run_reference_arm(args, cfg: dict, workload: dict) -> None:
         return
     nthreads = len(os.sched_getaffinity(0))
     world = int(os.environ.get("WORLD_SIZE", "1"))
-    g = cpu_graph_stack(cfg, nthreads)
+    try:
+        g = cpu_graph_stack(cfg, nthreads)
+    except FileNotFoundError as e:  # the reference's library is built from its tree
+        print(json.dumps({"impl": "reference", "unavailable": str(e)}), flush=True)
+        return
     x = np.random.default_rng(X_SEED).standard_normal(cfg["n_embd"]).astype(np.float32)
     for _ in range(args.warmup):
         g.decode(x, KV_POS, nthreads, logits=False)
@@ -636,16 +640,20 @@ def main() -> None:
     if rank == 0 and world == 1 and not args.no_cpu_baseline:
         # the reference's CPU step (its ggml graph on its ggml CPU backend),
         # bounded to ~12 s of steps, plus the three config-1 legs
-        g = cpu_graph_stack(cfg_d, nthreads)
-        g.decode(x_host, KV_POS, nthreads, logits=False)  # warm the caches of the CPU path
-        sec, n = time_cpu_steps(g, x_host, KV_POS, nthreads, 50, budget_s=12.0)
-        g.close()
-        cpu_baseline = {"value": round(step_bytes_of(cfg_d) / sec / 1e9, 3), "unit": "GB/s", "cores": nthreads,
-                        "kind": "reference", "tokens_per_s": round(1.0 / sec, 3), "cpu": cpu_model(),
-                        "sample": f"{n} full decode steps ({cfg_d['n_layer']} layers + LM head) of the reference "
-                                  f"engine's ggml graph on the reference's ggml CPU backend in ~12 s, {nthreads} "
-                                  f"threads; host-generated weights, {min(4, cfg_d['n_layer'])} distinct layers cycled",
-                        "legs": cpu_legs(nthreads)}
+        try:
+            g = cpu_graph_stack(cfg_d, nthreads)
+        except FileNotFoundError as e:  # the reference's library is built from its tree
+            cpu_baseline = {"unavailable": str(e)}
+        else:
+            g.decode(x_host, KV_POS, nthreads, logits=False)  # warm the caches of the CPU path
+            sec, n = time_cpu_steps(g, x_host, KV_POS, nthreads, 50, budget_s=12.0)
+            g.close()
+            cpu_baseline = {"value": round(step_bytes_of(cfg_d) / sec / 1e9, 3), "unit": "GB/s", "cores": nthreads,
+                            "kind": "reference", "tokens_per_s": round(1.0 / sec, 3), "cpu": cpu_model(),
+                            "sample": f"{n} full decode steps ({cfg_d['n_layer']} layers + LM head) of the reference "
+                                      f"engine's ggml graph on the reference's ggml CPU backend in ~12 s, {nthreads} "
+                                      f"threads; host-generated weights, {min(4, cfg_d['n_layer'])} distinct layers cycled",
+                            "legs": cpu_legs(nthreads)}
 
     if rank == 0:
         line = {
